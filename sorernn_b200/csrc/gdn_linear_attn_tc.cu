@@ -2,15 +2,17 @@
 //
 // One CTA per (value head, piece), 128 tokens a chunk. Per chunk, with A, B, C the roles' tiles and X the state:
 //   P  = A B^T                       (M = 128 tokens, N = 128 tokens, K = DB)
-//   Oi = A X                         (K = DB)
+//   Oi = A (Xhi + Xlo)               (K = DB; X split into two bf16)
 //   U^T = C^T (hi + lo)              (M = DC, N = DB, K = 128 tokens; hi + lo = su a^(..) B split into two bf16)
 //   Oa = (Whi + Wlo) C               (W(P): in-chunk decay, mask and scale, split into two bf16 in tensor memory)
 //   out = Oa + si a^(..) Oi          one rounding
 //   X <- a^nv X + U                  (fp32, in registers)
-// Roundings to bf16: X once, as Oi's operand, on top of the output's own (0.002 of RMS with it, 0.0017 without; where heads
-// never decay, the worst of a million outputs was off by 0.018 of RMS beyond its own rounding); A, B and C are exact, the
-// two-term splits of W(P) and of the state's operand are good to 2^-17. A caller that gets the state itself (final state,
-// gradient of the initial state) has it split in three (`precise`): fp32 accuracy.
+// A, B and C are exact; the two-term splits of X, of W(P) and of the state's operand are good to 2^-17, so outputs are
+// within 2e-4 of RMS of their own rounding however slowly a head decays (X in one term left up to 0.018 of RMS more; its
+// second term costs the seventh product: a scan of the shape below 121 -> 141 us). A caller that gets the state itself
+// (final state, gradient of the initial state) has its operand split in three (`precise`): fp32 accuracy. Two terms of a
+// 128 x 128 X do not fit beside the other tiles: its halves along DB, 32 KB of both terms, take turns in one place (the
+// staging tile in its stead, with outputs stored directly, made that 158 us).
 //
 // Keeping X in registers and U in an accumulator of its own takes the state off the tensor pipe's critical path: U of
 // a chunk needs nothing of the chunk before. 20 warps, handed over by mbarriers with bounded waits:
@@ -21,7 +23,7 @@
 //   warps 12-15  the state: thread = a row of X^T, 128 fp32 registers (registers moved here with setmaxnreg)
 //   warps 16, 18, 19  issue the MMAs (P and Oa; U; Oi), each in uniform control flow with the issue predicated
 //   warp 17      issues the loads (single buffers; L2 prefetch two chunks ahead)
-// 8 x 4,096 tokens x 16 heads, DB = DC = 128: a scan takes 122 us, 3.8 us a chunk, 0.67 of a copy's rate over the four
+// 8 x 4,096 tokens x 16 heads, DB = DC = 128: a scan takes 141 us, 4.4 us a chunk, 0.58 of a copy's rate over the four
 // tensors that it reads and writes; bound by the hand-overs between the roles and the products' shared-memory reads. The
 // fp32-accuracy kernel (gdn_linear_attn_simt.cu) takes 903 us (64 features: 417 against 90; one chunk of 16 heads: 36
 // against 25 with the call), so bf16 runs here at every size that this one supports. The states-only form runs the split,
@@ -29,7 +31,7 @@
 // of 65,536 tokens x 16 heads with one buffer and half a chunk ahead, 118 so). What decided the layout with outputs,
 // measured in the shape above (forward):
 //   * each role runs its code once a chunk, so the chunk loops have to fit the instruction cache together: 168 KB of
-//     unrolled code 12,800 cycles a chunk, 89 KB 6,900;
+//     unrolled code 12,800 cycles a chunk, 89 KB 6,900 (X in one term; X's terms written in two passes, 100 KB: 197 us);
 //   * an M = N = 128 product with both operands in shared memory takes nearly all of its read bandwidth (one every 65
 //     cycles): beside it a shared load of a warp's 512 bytes takes 60 cycles, a store 7, a global load 8. So the split
 //     reads B from global memory (L2) and the weights stay in registers.
@@ -82,10 +84,15 @@ struct Smem {
     static constexpr uint32_t LO2 = HI + NS * 2 * TB;  // third term of a precise split, else the output's staging tile
     static constexpr uint32_t ST = LO2;
     static constexpr uint32_t A = LO2 + (TB > TC ? TB : TC);
-    static constexpr uint32_t X = A + (OUT ? TB : 0);  // [DC rows][DB], DB / 64 blocks
-    static constexpr uint32_t TAB = X + (OUT ? DB / 64 * DC * 128 : 0);
+    // X^T: per 64 columns of DB a block [DC rows][64] of the high terms and one of the low ones; where there is room for
+    // 64 columns only (128 by 128 features), the two halves in turn in the same place
+    static constexpr uint32_t X = A + (OUT ? TB : 0);
+    static constexpr uint32_t BX = DC * 128;
+    static constexpr bool TURNS = DB == 128 && DC == 128;
+    static constexpr uint32_t NX = TURNS ? 2 : DB / 64 * 2;  // blocks
+    static constexpr uint32_t TAB = X + (OUT ? NX * BX : 0);
     static constexpr uint32_t BAR = TAB + 132 * 4;
-    static constexpr uint32_t INFO = BAR + 16 * 8;  // NBAR barriers and the TMEM address
+    static constexpr uint32_t INFO = BAR + 16 * 8;  // NBAR barriers
     static constexpr uint32_t RED = INFO + sizeof(Info);
     static constexpr uint32_t END = RED + (NTHR / 32 + 3) * 8;
     // more than half of an SM's shared memory, so that one CTA holds the SM's tensor memory
@@ -93,7 +100,9 @@ struct Smem {
 };
 static_assert(Smem<128, 128, true>::BYTES <= 232448 && Smem<128, 128, false>::BYTES <= 232448, "shared memory budget");
 
-enum Bar { FULL_A, FULL_B, FULL_C0, FULL_C1, QK, U, AX, O, HL, XR, UR, P0, P1, E, NBAR };
+// XR: X is written, AX: it has been multiplied. Where its halves take turns XR and AH are of the first, X2 and AX of the
+// second one.
+enum Bar { FULL_A, FULL_B, FULL_C0, FULL_C1, QK, U, AX, AH, O, HL, XR, X2, UR, P0, P1, E, NBAR };
 // Without outputs the split, its product and the product's accumulator have two buffers, and a barrier each, by chunk
 enum Bar2 { U_ODD = AX, HL_ODD = XR, UR_ODD = P0 };
 }  // namespace tk
@@ -425,13 +434,21 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                 wait(FULL_A, c);  // every phase in turn, also where nothing is issued
                 wait(XR, c);
                 if (c > 0) wait(E, c - 1);  // the outputs of chunk c - 1 have left Oi
-                if (c > 0 || has_x) {
+#pragma unroll 1
+                for (uint32_t half = 0; half < DB / 64; ++half) {
+                    if (S::TURNS && half) {
+                        commit_if(one, at(AH));
+                        wait(X2, c);
+                    }
+                    if (c == 0 && !has_x) continue;
                     tc_fence_after();
+#pragma unroll 1
+                    for (uint32_t term = 0; term < 2; ++term) {
+                        const uint32_t da = dA + half * (BLK >> 4);
+                        const uint32_t d = dX + ((S::TURNS ? 0 : half * 2) + term) * (S::BX >> 4);
 #pragma unroll
-                    for (int ks = 0; ks < DB / 16; ++ks) {
-                        const uint32_t o = (ks & 3) * 32;
-                        mma_if(one, tm + T_OI, dA + (((ks >> 2) * BLK + o) >> 4),
-                               dX + (((ks >> 2) * (DC * 128) + o) >> 4), id_x, ks);
+                        for (int ks = 0; ks < 4; ++ks)
+                            mma_if(one, tm + T_OI, da + ks * 2, d + ks * 2, id_x, half | term | ks);
                     }
                 }
                 commit_if(one, at(AX));
@@ -455,17 +472,30 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
 #pragma unroll
         for (int j = 0; j < XC; j += 2)
             x[j / 2] = from ? make_float2(src[j * ss], src[(j + 1) * ss]) : make_float2(0.f, 0.f);
-        auto write_x = [&]() {  // X^T tile: row = feature of C, DB along the row
-            if (OUT && live) {
-                uint8_t* const dst = sm + S::X + row * 128;
+        auto write_x = [&](int c) {  // X^T: row = feature of C, DB along the row
 #pragma unroll
-                for (int j = 0; j < DB; j += 8)
-                    *reinterpret_cast<uint4*>(dst + (j >> 6) * (DC * 128) + (((j >> 3) ^ row) & 7) * 16) =
-                        make_uint4(pack2(x[j / 2].x, x[j / 2].y), pack2(x[j / 2 + 1].x, x[j / 2 + 1].y),
-                                   pack2(x[j / 2 + 2].x, x[j / 2 + 2].y), pack2(x[j / 2 + 3].x, x[j / 2 + 3].y));
+            for (int j = 0; j < DB; j += 8) {
+                if (S::TURNS && j == 64) {
+                    fence_async_smem();
+                    arrive(XR);
+                    wait(AH, c);
+                }
+                if (live) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 y = x[(j / 2 + k) % (XC / 2)];
+                        hi[k] = pack2(y.x, y.y);
+                        lo[k] = pack2(y.x - lo_f(hi[k]), y.y - hi_f(hi[k]));
+                    }
+                    uint8_t* const dst = sm + S::X + (S::TURNS ? 0 : (j >> 6) * 2) * S::BX + row * 128 +
+                                         (((j >> 3) ^ row) & 7) * 16;
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(dst + S::BX) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
             }
             fence_async_smem();
-            arrive(XR);
+            arrive(S::TURNS ? X2 : XR);
         };
         const int nch = info->nch, n_u = info->n_u;
         const uint32_t tu0 = info->tm + lb + x0c;
@@ -490,7 +520,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
             }
             if (OUT && c + 1 < nch) {
                 if (c >= 0) wait(AX, c);  // X of this chunk has been read
-                write_x();
+                write_x(c + 1);
             }
         }
         float* dst = OUT ? (info->last ? a.x1 : nullptr) : a.local;

@@ -1,0 +1,71 @@
+"""Accuracy of linear attention's 16-bit outputs and gradients beyond their own rounding, against the token-by-token
+recurrence in 64 bits.
+
+What is measured is |got - ref| less half a unit in the last place of the output's type at ref (a correctly rounded result
+has none left), in units of RMS(ref). Bars, from the arithmetic:
+  * the tensor-memory kernel (bf16, head sizes 64 and 128) splits every operand that is not exact in bf16 (in-chunk
+    weights, keys times decay, the state) into two terms: 2^-18 of a value is lost, three such operands reach an output,
+    each an independent error on every term of a sum whose terms have random signs: sqrt(3) 2^-18 / sqrt(3) = 3.8e-6 of
+    the sum's own RMS. An element may be of a head whose RMS is 1.6 times that of all heads, late in a sequence whose RMS
+    grows by sqrt(2), and five and a half standard deviations off (a million values): 5e-5; its fp32 sums add as much
+    again: 2e-4 with a factor of two to spare.
+"""
+import numpy as np
+import pytest
+import torch
+
+from helpers import PARITY_LOG, CURRENT_TEST, rms
+from test_gpu_linear_attention import decays, inputs, oracle
+
+pytestmark = pytest.mark.gpu
+
+TC_TOL = 2e-4
+DIGITS = {torch.bfloat16: (8, -126), torch.float16: (11, -14)}  # significant bits, least exponent
+
+
+def excess(got, ref):
+    """max(|got - ref| - half an ulp of got's type at ref) / RMS(ref)"""
+    r = ref.double().cpu().numpy()
+    a = got.detach().double().cpu().numpy()
+    assert a.shape == r.shape and np.isfinite(a).all()
+    bits, least = DIGITS[got.dtype]
+    _, e = np.frexp(r)  # |r| in [2^(e-1), 2^e)
+    half = np.exp2(np.maximum(e - 1, least).astype(np.float64) - bits)
+    return float((np.abs(a - r) - half).max()) / max(rms(r), 1e-30)
+
+
+def within(name, got, ref, tol):
+    x = excess(got, ref)
+    PARITY_LOG.append((name, x, x, tol, CURRENT_TEST[0]))
+    assert x <= tol, f"{name}: {x:.3e} of RMS beyond the output's rounding, bar {tol}"
+
+
+def run(B, T, H, HV, K, V, dtype, decay, tol, cu=None, state=True, seed=0):
+    from sorernn_b200 import chunk_linear_attention
+
+    N = B if cu is None else len(cu) - 1
+    x = inputs(B, T, H, HV, K, V, dtype, N, state, seed)
+    ld = decays(HV, decay)
+    leaves = [x[n].requires_grad_(True) for n in ("q", "k", "v")]
+    cu_t = None if cu is None else torch.tensor(cu, device="cuda")
+    o, ht = chunk_linear_attention(x["q"], x["k"], x["v"], ld, initial_state=x["h0"], output_final_state=True,
+                                   cu_seqlens=cu_t, cu_seqlens_cpu=None if cu is None else cu_t.cpu())
+    outs, cots = ((o, ht), (x["do"], x["dht"])) if state else ((o,), (x["do"],))
+    grads = torch.autograd.grad(outs, leaves, cots)
+    ref = oracle(x["q"], x["k"], x["v"], ld, K ** -0.5, cu, x["h0"], x["do"], x["dht"])
+    for n, y in zip(("o", "dq", "dk", "dv"), (o,) + grads):
+        within("lin 16-bit " + n, y, ref[n], tol)
+
+
+@pytest.mark.parametrize("K,V", [(128, 128), (64, 64), (64, 128), (128, 64)])
+@pytest.mark.parametrize("decay", ["slopes", "edges"])
+def test_tensor_memory_kernel_whole_sequences(K, V, decay):
+    """Many pairs, several chunks each: nothing is cut."""
+    run(16, 300, 10, 10, K, V, torch.bfloat16, decay, TC_TOL, seed=11)
+
+
+@pytest.mark.parametrize("K,V", [(128, 128), (64, 64), (64, 128), (128, 64)])
+@pytest.mark.parametrize("T", [1900, 1920])
+def test_tensor_memory_kernel_cut_sequences(K, V, T):
+    """Pieces side by side, heads that never decay and heads that decay at once: the state enters every output."""
+    run(2, T, 5, 5, K, V, torch.bfloat16, "edges", TC_TOL, seed=6)
