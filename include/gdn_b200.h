@@ -26,8 +26,8 @@
  *    cu_seqlens[i] (gdn_ref.py:53-61); without it every batch row is one sequence (N = B).
  *  - the caller allocates every output and the workspace (size from the *_workspace_size query);
  *    the library never allocates device memory. Its only device state: one 4-byte error word per
- *    workspace-less streaming kernel family (decode, norm-gate, conv) and linear attention (see gdn_stream_kernels_error)
- *    and the fixed scratch array of gdn_chunk_bwd_noalloc.
+ *    workspace-less streaming kernel family (decode, norm-gate, conv) and for linear attention (see
+ *    gdn_stream_kernels_error), and the fixed scratch array of gdn_chunk_bwd_noalloc.
  *  - every call is stream-ordered on `stream`, does not synchronise the host, and returns a status
  *    code (GDN_OK = 0); nothing aborts or traps. Shapes, dtypes and alignment are checked on the host
  *    before any launch.
@@ -393,9 +393,10 @@ int gdn_qk_norm_rope_bwd(const gdn_qk_norm_rope_problem* p, const void* q, const
 int gdn_workspace_error(const void* workspace, gdn_stream_t stream, int32_t* error_out);
 
 /* Reads and clears the device error words of the workspace-less streaming kernels (gdn_decode_step,
- * the norm-gate and conv entry points) and of gdn_linear_attn_fwd / _bwd on the current device: 0 = none, else the code of the first
- * kernel family whose bounded stage wait gave up (31 decode, 32 norm-gate, 33 conv, 34 linear attention). A kernel that gave
- * up stores nothing from then on (the decode step leaves those states unchanged). Synchronises `stream`.
+ * the norm-gate and conv entry points) and of gdn_linear_attn_fwd / _bwd on the current device: 0 = none, else
+ * the code of the first kernel family whose bounded stage wait gave up (31 decode, 32 norm-gate, 33 conv, 34
+ * linear attention). A kernel that gave up stores nothing from then on (the decode step leaves those states
+ * unchanged; of a linear attention call, what was not stored is undefined). Synchronises `stream`.
  * No counterpart in the reference. */
 int gdn_stream_kernels_error(gdn_stream_t stream, int32_t* error_out);
 

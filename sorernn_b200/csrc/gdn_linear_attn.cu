@@ -80,8 +80,8 @@ static ScanPlan plan(const gdn_linear_attn_problem* p, int64_t DB, int64_t DC, i
     s.tc = scan_tc_supported(DB, DC, p->act_dtype);
     s.chunk = s.tc ? kTcChunk : kSimtChunk;
     const int64_t sms = device_sm_count();
-    // measured: a chunk 4.4 us (128 tokens, tensor cores), start-up 5.7, states-only chunk 2.1, the two more launches 7
-    const PieceCost cost = s.tc ? PieceCost{sms, 1.3, 0.48, 1.6, 0.1}
+    // measured: a chunk 4.7 us (128 tokens, tensor cores), start-up 5.7, states-only chunk 2.1, the two more launches 7
+    const PieceCost cost = s.tc ? PieceCost{sms, 1.2, 0.45, 1.5, 0.1}
                                 : PieceCost{sms * (DB <= 64 && DC <= 64 ? 2 : 1), 0.5, 0.6, 1.8, 0.1};
     s.piece_chunks = choose_piece_chunks(p, s.chunk, p->HV * n_scans, cost);
     const int64_t per = (int64_t)s.chunk * s.piece_chunks;

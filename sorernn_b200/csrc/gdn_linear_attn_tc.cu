@@ -23,7 +23,7 @@
 //   warps 12-15  the state: thread = a row of X^T, 128 fp32 registers (registers moved here with setmaxnreg)
 //   warps 16, 18, 19  issue the MMAs (P and Oa; U; Oi), each in uniform control flow with the issue predicated
 //   warp 17      issues the loads (single buffers; L2 prefetch two chunks ahead)
-// 8 x 4,096 tokens x 16 heads, DB = DC = 128: a scan takes 141 us, 4.4 us a chunk, 0.58 of a copy's rate over the four
+// 8 x 4,096 tokens x 16 heads, DB = DC = 128: a scan takes 149 us, 4.7 us a chunk, 0.55 of a copy's rate over the four
 // tensors that it reads and writes; bound by the hand-overs between the roles and the products' shared-memory reads. The
 // fp32-accuracy kernel (gdn_linear_attn_simt.cu) takes 903 us (64 features: 417 against 90; one chunk of 16 heads: 36
 // against 25 with the call), so bf16 runs here at every size that this one supports. The states-only form runs the split,
@@ -69,7 +69,7 @@ struct Info {
     int nch, n_u;             // chunks; chunks whose U is formed
     int last, has_x;          // the piece that leaves the sequence; a state comes in
     uint32_t tm;              // tensor memory
-    int pad;
+    int failed;               // a warp of the outputs' role gave up
 };
 
 template <int DB, int DC, bool OUT>
@@ -92,7 +92,7 @@ struct Smem {
     static constexpr uint32_t NX = TURNS ? 2 : DB / 64 * 2;  // blocks
     static constexpr uint32_t TAB = X + (OUT ? NX * BX : 0);
     static constexpr uint32_t BAR = TAB + 132 * 4;
-    static constexpr uint32_t INFO = BAR + 16 * 8;  // NBAR barriers
+    static constexpr uint32_t INFO = BAR + 20 * 8;  // NBAR barriers
     static constexpr uint32_t RED = INFO + sizeof(Info);
     static constexpr uint32_t END = RED + (NTHR / 32 + 3) * 8;
     // more than half of an SM's shared memory, so that one CTA holds the SM's tensor memory
@@ -102,7 +102,9 @@ static_assert(Smem<128, 128, true>::BYTES <= 232448 && Smem<128, 128, false>::BY
 
 // XR: X is written, AX: it has been multiplied. Where its halves take turns XR and AH are of the first, X2 and AX of the
 // second one.
-enum Bar { FULL_A, FULL_B, FULL_C0, FULL_C1, QK, U, AX, AH, O, HL, XR, X2, UR, P0, P1, E, NBAR };
+// D16, D18, D19: all products of an issuing warp are done (once, at its end).
+enum Bar { FULL_A, FULL_B, FULL_C0, FULL_C1, QK, U, AX, AH, O, HL, XR, X2, UR, P0, P1, E, D16, D18, D19, NBAR };
+static_assert(NBAR <= 20, "barriers");
 // Without outputs the split, its product and the product's accumulator have two buffers, and a barrier each, by chunk
 enum Bar2 { U_ODD = AX, HL_ODD = XR, UR_ODD = P0 };
 }  // namespace tk
@@ -165,8 +167,11 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
 }
 // Barriers by their shared-memory address (a handful of instructions a use: see the note on the instruction cache).
 // A bounded wait: `left` polls remain to the thread (a poll that fails suspends for microseconds, so the budget is
-// about a second, where a chunk takes four microseconds); once they are spent every later wait looks once, so the CTA
-// runs out.
+// about a second, where a chunk takes four microseconds); once they are spent, `left` stays 1 and every later wait looks
+// once. A warp that gave up hands over and stores nothing from then on, nor writes what a product or a copy may still read:
+// the roles end their loops, but for the outputs' one, which meets in named barriers and runs out. So the others give up in
+// their turn, no barrier gets an arrival that it does not expect, and what reaches memory was made from complete operands.
+// The warps that issue loads and products wait for theirs before the CTA gives its memory back.
 constexpr uint32_t kPolls = 1u << 19;
 __device__ __forceinline__ void wait_at(uint32_t bar, uint32_t parity, uint32_t& left) {
     asm volatile(
@@ -276,11 +281,12 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
             info->nch = nch;
             info->n_u = !OUT || (last && a.x1) ? nch : nch - 1;  // the last chunk's only if its end state is wanted
             info->last = last;
+            info->failed = 0;
             info->has_x = OUT && (a.x0 || (a.local && (a.reverse ? p < pieces - 1 : p > 0)));
         }
     }
     if (tid == 16 * 32) {
-        for (int i = 0; i < NBAR; ++i) mbar_init(&bar[i], i >= P0 || (!OUT && i >= HL) ? 8 : i >= HL ? 4 : 1);
+        for (int i = 0; i < NBAR; ++i) mbar_init(&bar[i], i >= D16 ? 1 : i >= P0 || (!OUT && i >= HL) ? 8 : i >= HL ? 4 : 1);
         fence_barrier_init();
     }
     if (tid == 17 * 32) {
@@ -306,9 +312,18 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
     auto odd = [&](int c) { return OUT ? 0u : (uint32_t)c & 1u; };
     constexpr int AHEAD = S::NS;  // buffers of those three
     auto wait_c = [&](int c) { wait(FULL_C0 + (S::NC == 2 ? c & 1 : 0), S::NC == 2 ? c >> 1 : c); };
+    auto gave_up = [&]() { return __any_sync(0xffffffffu, polls == 1) != 0; };
     auto arrive = [&](int b) {
+        const bool go = !gave_up();
         __syncwarp();
-        if (lane == 0) arrive_at(at(b));
+        if (go && lane == 0) arrive_at(at(b));
+    };
+    // the end of a warp that issues products: they are done
+    auto drain = [&](int b) {
+        uint32_t left = kPolls;
+        commit_if(lane == 0, at(b));
+        wait_at(at(b), 0, left);
+        tc_fence_after();
     };
     // whether the chunk that starts at t has its split in three terms (see Info)
     auto precise_at = [&](int t) { return PRECISE && (a.reverse ? t - info->bos : info->eos - t - C) < info->n_precise; };
@@ -317,6 +332,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
     // zeros in C's rows past the end, by 128 threads
     auto zero_tail = [&](int c, int nv, int t) {
         wait_c(c);
+        if (gave_up()) return;
         uint8_t* ct = sm + S::Ct + (S::NC == 2 ? (c & 1) * S::TC : 0);
         for (int e = nv * 8 + t; e < C * 8; e += 128)
 #pragma unroll
@@ -328,7 +344,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
         if (warp == 17 && lane == 0) {
             const int hA = hv / a.gA, hB = hv / a.gB, hC = hv / a.gC;
             const int nch = info->nch, tok_step = info->tok_step;
-            int t = info->tok_first;
+            int t = info->tok_first, loaded[3] = {0, 0, 0};  // loads issued of A, B, C
 #pragma unroll 1
             for (int c = 0; c < nch; ++c, t += tok_step) {
                 auto load = [&](const CUtensorMap* map, uint32_t dst, int b, int h, uint32_t bytes) {
@@ -338,9 +354,13 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                 };
                 if (OUT) {
                     if (c > 0) wait(QK, c - 1);
+                    if (polls == 1) break;
                     load(&args.tB, S::B, FULL_B, hB, S::TB);
+                    ++loaded[1];
                     if (c > 0) wait(AX, c - 1);
+                    if (polls == 1) break;
                     load(&args.tA, S::A, FULL_A, hA, S::TB);
+                    ++loaded[0];
                     if (c > 0) {  // U and Oa of chunk c - 1 have read C
                         wait(U, c - 1);
                         wait(O, c - 1);
@@ -348,8 +368,10 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                 } else if (c > 1) {
                     wait_u(c - 2);  // it has read this buffer of C
                 }
+                if (polls == 1) break;
                 const int cb = S::NC == 2 ? c & 1 : 0;
                 load(&args.tC, S::Ct + cb * S::TC, FULL_C0 + cb, hC, S::TC);
+                ++loaded[2];
                 for (int d = c ? c + 2 : 1; d <= c + 2 && d < nch; ++d)  // to L2, two chunks ahead
                     for (int kb = 0; kb < (DB > DC ? DB : DC); kb += 64) {
                         const int td = t + (d - c) * tok_step;
@@ -357,6 +379,13 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                         if (kb < DB) prefetch_tile_l2(&args.tB, kb, hB, td);
                         if (kb < DC) prefetch_tile_l2(&args.tC, kb, hC, td);
                     }
+            }
+            uint32_t left = kPolls;  // the last load of each barrier has landed
+            if (loaded[0] > 0) wait_at(at(FULL_A), (loaded[0] - 1) & 1, left);
+            if (loaded[1] > 0) wait_at(at(FULL_B), (loaded[1] - 1) & 1, left);
+            for (int b = 0; b < (int)S::NC; ++b) {
+                const int n = (loaded[2] + (int)S::NC - 1 - b) / (int)S::NC;
+                if (n > 0) wait_at(at(FULL_C0 + b), (n - 1) & 1, left);
             }
         } else if (OUT && warp == 16) {
             const uint32_t one = lane == 0;
@@ -369,6 +398,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                 wait(FULL_A, c);
                 wait(FULL_B, c);
                 if (c > 0) wait(O, c - 1);  // W(P) of chunk c - 1 has been read
+                if (gave_up()) break;
                 tc_fence_after();
 #pragma unroll
                 for (int ks = 0; ks < DB / 16; ++ks) {
@@ -381,6 +411,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
 #pragma unroll 1
                 for (uint32_t half = 0; half < 2; ++half) {
                     wait(half ? P1 : P0, c);
+                    if (gave_up()) break;
                     tc_fence_after();
 #pragma unroll 1
                     for (uint32_t lo = 0; lo < 2; ++lo) {
@@ -391,8 +422,10 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                                       half | lo | ks);
                     }
                 }
+                if (gave_up()) break;
                 commit_if(one, at(O));
             }
+            drain(D16);
         } else if (warp == 18) {
             const uint32_t one = lane == 0;
             constexpr uint32_t id_u = idesc_bf16(128, DB, 1, 1);
@@ -407,6 +440,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                 wait_c(c);
                 wait_hl(c);
                 if (c >= AHEAD) wait_ur(c - AHEAD);
+                if (gave_up()) break;
                 if (c < n_u) {
                     tc_fence_after();
                     const uint32_t terms = precise_at(t) ? 3 : 2;
@@ -422,6 +456,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                 }
                 commit_if(one, at(odd(c) ? (int)U_ODD : (int)U));
             }
+            drain(D18);
         } else if (OUT && warp == 19) {
             const uint32_t one = lane == 0;
             constexpr uint32_t id_x = idesc_bf16(128, DC, 0, 0);
@@ -440,6 +475,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                         commit_if(one, at(AH));
                         wait(X2, c);
                     }
+                    if (gave_up()) break;
                     if (c == 0 && !has_x) continue;
                     tc_fence_after();
 #pragma unroll 1
@@ -451,8 +487,10 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                             mma_if(one, tm + T_OI, da + ks * 2, d + ks * 2, id_x, half | term | ks);
                     }
                 }
+                if (gave_up()) break;
                 commit_if(one, at(AX));
             }
+            drain(D19);
         }
     } else if (OUT ? warp >= 12 : warp < 8) {
         // ---- the state ----
@@ -479,6 +517,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                     fence_async_smem();
                     arrive(XR);
                     wait(AH, c);
+                    if (gave_up()) return;
                 }
                 if (live) {
                     uint32_t hi[4], lo[4];
@@ -505,6 +544,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                 const float f = pw[tokens_at(info->tok_first + c * info->tok_step)];
                 const uint32_t tu = tu0 + (odd(c) ? T_P : T_U);
                 wait_u(c);
+                if (gave_up()) break;
                 tc_fence_after();
 #pragma unroll
                 for (int j = 0; j < XC; j += 16) {
@@ -520,10 +560,12 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
             }
             if (OUT && c + 1 < nch) {
                 if (c >= 0) wait(AX, c);  // X of this chunk has been read
+                if (gave_up()) break;
                 write_x(c + 1);
             }
         }
         float* dst = OUT ? (info->last ? a.x1 : nullptr) : a.local;
+        if (gave_up()) dst = nullptr;
         if (dst && live) {
             dst += OUT ? xrow : lrow;
             const int ds = OUT ? xs : DC;
@@ -552,7 +594,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
         // the rows' factors, as fp32 (precise) or as a pair of bf16, f = fh + fl
         uint32_t fx[NR];
         int nv = -1;
-        bool prec = false;
+        bool prec = false, good = true;
         const int nch = info->nch, n_u = info->n_u, tok_first = info->tok_first, tok_step = info->tok_step;
         constexpr int NB = DB / 64;
 #pragma unroll 1
@@ -579,13 +621,14 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                 if (c >= AHEAD) wait_u(c - AHEAD);
                 if (PRECISE && !OUT && prec && c > 0) wait_u(c - 1);  // the third term has one buffer
                 if (!OUT) wait_c(c);  // every phase in turn
+                good = !gave_up();
                 if (nv < C) zero_tail(c, nv, t4 & 127);
             }
             // each row's registers are loaded again as soon as they are used
             const int next = (step + DEPTH) / NB;
             const int tn = tok_first + next * tok_step, rows = next < n_u ? tokens_at(tn) : 0;
             const __nv_bfloat16* src = b0 + (tn + r0) * bstep + (step + DEPTH) % NB * 64;
-            if (c < n_u) {
+            if (c < n_u && good) {
                 uint8_t* const dst1 = dst0 + odd(c) * (2 * S::TB) + kb * BLK;
 #pragma unroll
                 for (int i = 0; i < NR; ++i, src += RS * bstep) {
@@ -651,7 +694,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
             const bool fast = g >= -5.f, wide = ((uintptr_t)a.out & 31) == 0;
 #pragma unroll 1
             for (int c = 0; c < nch; ++c, t0 += tok_step) {
-                const int nv = min(eos - t0, C);
+                int nv = min(eos - t0, C);
                 const int m_end = a.reverse ? nv : C;  // forward: m <= r < nv leaves the tail out by itself
                 // A chunk whose split has a third term keeps it in the staging tile. The last tile before that is given
                 // up two chunks ahead, and read out before this chunk's W(P): Oa follows it, then the next chunk's U,
@@ -735,6 +778,10 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                 }
                 if (inter) wait(AX, c);
                 wait(O, c);
+                if (gave_up()) {  // nothing of this chunk is stored, nor of a later one
+                    nv = 0;
+                    if (lane == 0) info->failed = 1;
+                }
                 tc_fence_after();
                 float x0[16], y0[16];
                 tmem_ld16(tm + T_OA + DC / 2 * h, x0);
@@ -779,7 +826,7 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
                 if (staged) {
                     fence_async_smem();
                     asm volatile("bar.sync 1, 256;" ::: "memory");
-                    if (tid == 0) {
+                    if (tid == 0 && !*(volatile int*)&info->failed) {
 #pragma unroll
                         for (int kb = 0; kb < DC / 64; ++kb)
                             tma_store_3d(&args.tO, sm + S::ST + kb * BLK, kb * 64, hv, t0);
