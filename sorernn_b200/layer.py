@@ -144,17 +144,21 @@ class LinearAttention(nn.Module):
             raise ValueError(f"log_decay must be v_heads = {v_heads} values <= 0")
         self._log_decay = [float(x) for x in log_decay]
         self._table_args = (max_positions, head_dim // 4 if rotary_dim is None else rotary_dim, theta)
-        self._constants(None)
+        for name, value in zip(("log_decay", "table"), self._constants(None)):
+            self.register_buffer(name, value, persistent=False)
 
-    def _constants(self, device: Optional[torch.device]) -> None:
-        self.register_buffer("log_decay", torch.tensor(self._log_decay, dtype=torch.float32, device=device),
-                             persistent=False)
-        self.register_buffer("table", rotary_table(*self._table_args, device=device), persistent=False)
+    def _constants(self, device: Optional[torch.device]) -> tuple[Tensor, Tensor]:
+        return (torch.tensor(self._log_decay, dtype=torch.float32, device=device),
+                rotary_table(*self._table_args, device=device))
 
     def _apply(self, fn, recurse: bool = True):
+        before = self.log_decay, self.table
         super()._apply(fn, recurse)
-        if self.table.dtype != torch.float32:  # a cast of the parameters: the constants stay fp32
-            self._constants(self.table.device)
+        if self.table is not before[1]:  # moved, cast or emptied, as after construction on the meta device: the
+            # constants keep their values, in fp32, and no checkpoint holds them
+            device = self.table.device
+            kept = self._constants(torch.device("cpu")) if before[1].is_meta else before
+            self.log_decay, self.table = (t.to(device) for t in kept)
         return self
 
     def _qkv(self, x: Tensor, positions: Tensor) -> tuple[Tensor, Tensor, Tensor]:

@@ -1,0 +1,43 @@
+"""Host-side checks of the linear-attention layer (no GPU)."""
+import pytest
+import torch
+
+from sorernn_b200.layer import LinearAttention
+
+ARGS = dict(d_model=64, qk_heads=1, v_heads=2, head_dim=32, max_positions=16)
+
+
+def constants(layer):
+    return layer.log_decay, layer.table
+
+
+@pytest.mark.parametrize("wrapped", [False, True])
+@pytest.mark.parametrize("dtype", [None, torch.bfloat16])
+@pytest.mark.parametrize("start", ["meta", "cpu"])
+def test_constants_survive_to_empty(start, dtype, wrapped):
+    """Built on the meta device, given memory and loaded from a checkpoint, which does not hold the constants; and
+    emptied in place."""
+    want = LinearAttention(**ARGS)
+    with torch.device(start):
+        layer = LinearAttention(**ARGS)
+    model = torch.nn.Sequential(layer) if wrapped else layer
+    if dtype is not None:
+        model.to(dtype)
+    model.to_empty(device="cpu")
+    layer.load_state_dict(want.state_dict(), strict=True)
+    for a, b in zip(constants(layer), constants(want)):
+        assert a.dtype == torch.float32 and a.device.type == "cpu" and torch.equal(a, b)
+    assert [n for n, _ in layer.named_buffers()] == ["log_decay", "table"] and "table" not in layer.state_dict()
+
+
+def test_constants_through_casts_and_moves():
+    layer = LinearAttention(**ARGS, log_decay=[-1.0, -0.25])
+    want = [t.clone() for t in constants(layer)]
+    table = layer.table
+    layer.to("cpu")
+    assert layer.table is table  # nothing to move
+    for move in (lambda m: m.bfloat16(), lambda m: m.double(), lambda m: m.to("meta"), lambda m: m.to_empty(device="cpu")):
+        move(layer)
+        assert layer.table.dtype == layer.log_decay.dtype == torch.float32
+        if not layer.table.is_meta:
+            assert all(torch.equal(a, b) for a, b in zip(constants(layer), want))
