@@ -114,7 +114,9 @@ class LinearAttention(nn.Module):
 
     ``forward(x [B,T,d_model], positions=None, cu_seqlens=None, cu_seqlens_cpu=None, initial_state=None,
     output_final_state=False)`` runs whole sequences (training, prefill): every batch row is a document, or with
-    ``cu_seqlens`` (int64 ``[N+1]``, B == 1) every packed span; positions default to the token's place in its document.
+    ``cu_seqlens`` (int64 ``[N+1]``, B == 1) every packed span; positions default to the token's place in its document,
+    counted from 0 also where ``initial_state`` continues one (give ``positions`` there). A document that is known on the
+    host to pass ``max_positions`` is refused; a position outside the table otherwise makes its outputs NaN.
     Returns y, or ``(y, state [N,v_heads,head_dim,head_dim])`` with ``output_final_state``.
     ``step(x [N,d_model], positions [N], state, state_indices=None)`` continues N requests by one token each on their
     fp32 states, updated in place (``linear_attention_step``); positions ``[axes,N]`` with ``sections``.
@@ -178,6 +180,12 @@ class LinearAttention(nn.Module):
                 output_final_state: bool = False):
         b, t, _ = x.shape
         if positions is None:
+            longest = t
+            if cu_seqlens is not None:  # known on the host if the lengths are
+                lengths = None if cu_seqlens_cpu is None else cu_seqlens_cpu[1:] - cu_seqlens_cpu[:-1]
+                longest = int(lengths.max()) if lengths is not None and lengths.numel() else 0
+            if longest > self.table.shape[0]:  # its rotated features would be NaN, and every token's after them
+                raise ValueError(f"a document of {longest} tokens is longer than max_positions = {self.table.shape[0]}")
             positions = torch.arange(t, device=x.device)
             if cu_seqlens is not None:  # the place in the document, without reading the lengths on the host
                 cu = cu_seqlens.to(x.device)

@@ -41,3 +41,22 @@ def test_constants_through_casts_and_moves():
         assert layer.table.dtype == layer.log_decay.dtype == torch.float32
         if not layer.table.is_meta:
             assert all(torch.equal(a, b) for a, b in zip(constants(layer), want))
+
+
+def test_documents_past_the_table_are_refused():
+    """16 positions: longer documents are refused before any kernel; shorter ones of a longer window, lengths that only
+    the device knows, and given positions go on (to the ops, which take no CPU tensors)."""
+    layer = LinearAttention(**ARGS)
+    x = torch.randn(1, 20, 64)
+    cu = torch.tensor([0, 3, 20])
+    with pytest.raises(ValueError, match="max_positions = 16"):
+        layer(x)
+    with pytest.raises(ValueError, match="document of 17 tokens"):
+        layer(x, cu_seqlens=cu, cu_seqlens_cpu=cu)
+    short = torch.tensor([0, 4, 20])
+    for kw in (dict(cu_seqlens=short, cu_seqlens_cpu=short), dict(cu_seqlens=cu),
+               dict(positions=torch.zeros(1, 20, dtype=torch.int64))):
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            layer(x, **kw)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        layer(x[:, :16])
