@@ -188,7 +188,7 @@ class LinearAttention(nn.Module):
                 raise ValueError(f"a document of {longest} tokens is longer than max_positions = {self.table.shape[0]}")
             positions = torch.arange(t, device=x.device)
             if cu_seqlens is not None:  # the place in the document, without reading the lengths on the host
-                cu = cu_seqlens.to(device=x.device, dtype=positions.dtype)
+                cu = cu_seqlens.to(x.device)
                 positions = positions - cu[torch.searchsorted(cu, positions, right=True) - 1]
             positions = positions.expand(b, t)
             if self.sections:

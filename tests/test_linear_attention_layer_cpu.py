@@ -60,11 +60,3 @@ def test_documents_past_the_table_are_refused():
             layer(x, **kw)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         layer(x[:, :16])
-
-
-@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
-def test_document_ends_of_either_width(dtype):
-    """The default positions take document ends of any integer type, as the scan itself does."""
-    layer = LinearAttention(**ARGS)
-    with pytest.raises(RuntimeError, match="CUDA tensors only"):  # past the positions, at the first op
-        layer(torch.randn(1, 12, 64), cu_seqlens=torch.tensor([0, 5, 12], dtype=dtype))
