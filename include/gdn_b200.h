@@ -348,7 +348,7 @@ int gdn_linear_attn_bwd(const gdn_linear_attn_problem* p, const void* q, const v
 /* One token for N requests on fp32 states [n_slots, HV, DK, DV], updated in place: q, k [N, H, DK], v, o [N, HV, DV].
  * slots (device int32 [N], or NULL: request n uses state n) names each request's state; the slots of one call are
  * distinct. A negative slot is an idle request: its o is zero and no state changes; a slot >= n_slots touches no
- * state either and gives NaN. */
+ * state either and gives NaN. The states have to be 16-byte aligned where DV is a multiple of 4; nothing else has. */
 int gdn_linear_attn_step(int64_t N, int64_t H, int64_t HV, int64_t DK, int64_t DV, float scale, int32_t act_dtype,
                          const void* q, const void* k, const void* v, const float* log_decay, float* state,
                          int64_t n_slots, const int32_t* slots, void* o, gdn_stream_t stream);

@@ -117,7 +117,7 @@ extern "C" int gdn_linear_attn_step(int64_t N, int64_t H, int64_t HV, int64_t DK
     if (act_dtype != GDN_BF16 && act_dtype != GDN_FP16 && act_dtype != GDN_FP32) return GDN_ERR_DTYPE;
     if (N == 0) return GDN_OK;
     if (!q || !k || !v || !log_decay || !o || (n_slots > 0 && !state)) return GDN_ERR_ARGUMENT;
-    if ((uintptr_t)state & 15) return GDN_ERR_ALIGN;
+    if (DV % 4 == 0 && ((uintptr_t)state & 15)) return GDN_ERR_ALIGN;  // rows of whole 16-byte vectors
     StepArgs a{};
     a.q = q; a.k = k; a.v = v; a.log_decay = log_decay; a.state = state; a.slots = slots; a.o = o;
     a.n_slots = n_slots;

@@ -28,6 +28,12 @@ def _at(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _aligned(t: Optional[Tensor]) -> Optional[Tensor]:
+    """``t`` (contiguous), or a copy where its memory starts off the library's 16-byte grid, as that of a slice may;
+    autograd hands such slices over as gradients, of a concatenation for instance."""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _call(device: torch.device, fn, name: str, *args) -> None:
     """One library call on ``device``'s current stream (the last argument of every entry point)."""
     index = device.index
@@ -52,6 +58,7 @@ def _problem(q: Tensor, v: Tensor, cu_seqlens: Optional[Tensor], scale: float,
 def _fwd(q, k, v, log_decay, initial_state, cu_seqlens, scale, max_seqlen, want_state):
     L = _lib.lib()
     p = _problem(q, v, cu_seqlens, scale, max_seqlen)
+    q, k, v, initial_state = _aligned(q), _aligned(k), _aligned(v), _aligned(initial_state)
     o = torch.empty_like(v)
     final = q.new_empty((p.N, p.HV, p.DK, p.DV), dtype=torch.float32) if want_state else None
     ref = ctypes.byref(p)
@@ -83,8 +90,9 @@ def _bwd(q, k, v, log_decay, initial_state, do, dht, cu_seqlens, scale, max_seql
     p = _problem(q, v, cu_seqlens, scale, max_seqlen)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     dh0 = q.new_empty((p.N, p.HV, p.DK, p.DV), dtype=torch.float32) if want_dh0 else None
-    do = do.contiguous()
-    dht = None if dht is None else dht.float().contiguous()
+    q, k, v, initial_state = _aligned(q), _aligned(k), _aligned(v), _aligned(initial_state)
+    do = _aligned(do.contiguous())
+    dht = None if dht is None else _aligned(dht.float().contiguous())
     ref = ctypes.byref(p)
     n = L.gdn_linear_attn_bwd_workspace_size(ref)
     ws = q.new_empty(n, dtype=torch.uint8) if n else None
@@ -223,6 +231,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     Without ``state_indices``, ``state`` is ``[N,HV,K,V]``. With ``state_indices`` (int32 ``[N]`` on the device, no two
     alike), ``state`` is a pool ``[slots,HV,K,V]`` and request n uses ``state[state_indices[n]]``; a negative index is
     an idle request (its output is zero, no state changes) and an index past the pool gives NaN and touches nothing.
+    Where V is a multiple of 4 the state's memory has to start on a 16-byte boundary.
     """
     if not q.is_cuda:
         raise RuntimeError("sorernn_b200 runs on CUDA tensors only (no CPU fallback)")

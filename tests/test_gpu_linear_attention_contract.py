@@ -32,3 +32,60 @@ def test_no_wait_runs_out(K, V, B, T, cu):
                                    cu_seqlens=None if cu is None else torch.tensor(cu, device="cuda"))
     torch.autograd.grad((o, ht), leaves, (x["do"], x["dht"]))
     assert error_word() == 0
+
+
+def off_grid(t):
+    """The values of t in contiguous memory that starts one element past a 16-byte boundary."""
+    buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    assert buf.data_ptr() % 16 == 0
+    return buf[1:].copy_(t.flatten()).view(t.shape)
+
+
+@pytest.mark.parametrize("dtype,K,V", [(torch.float32, 20, 33), (torch.float32, 64, 64), (torch.bfloat16, 128, 128),
+                                       (torch.float16, 7, 128)])
+def test_memory_off_the_16_byte_grid(dtype, K, V):
+    """Inputs, states and gradients of any alignment give what aligned ones do."""
+    from sorernn_b200 import chunk_linear_attention
+
+    x = inputs(2, 70, 1, 2, K, V, dtype, state=True, seed=4)
+    results = []
+    for move in (lambda t: t.clone(), off_grid):
+        y = {n: move(t) for n, t in x.items()}
+        leaves = [y[n].requires_grad_(True) for n in ("q", "k", "v", "h0")]
+        o, ht = chunk_linear_attention(y["q"], y["k"], y["v"], decays(2), initial_state=y["h0"], output_final_state=True)
+        results.append([o, ht, *torch.autograd.grad((o, ht), leaves, (y["do"], y["dht"]))])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_gradient_of_a_concatenation():
+    """The second part's gradient is a slice of the whole's, at byte 37 x 33 x 4 of its memory."""
+    from sorernn_b200 import chunk_linear_attention
+
+    a, b = (inputs(1, T, 1, 1, 20, 33, torch.float32, seed=5) for T in (37, 22))
+    leaves = [y[n].requires_grad_(True) for y in (a, b) for n in ("q", "k", "v")]
+    parts = [chunk_linear_attention(y["q"], y["k"], y["v"], decays(1))[0] for y in (a, b)]
+    got = torch.autograd.grad(torch.cat(parts, 1), leaves, torch.cat([a["do"], b["do"]], 1))
+    want = torch.autograd.grad(parts_again(a, b), leaves, (a["do"], b["do"]))
+    for u, w in zip(got, want):
+        assert torch.equal(u, w)
+
+
+def parts_again(a, b):
+    from sorernn_b200 import chunk_linear_attention
+
+    return [chunk_linear_attention(y["q"], y["k"], y["v"], decays(1))[0] for y in (a, b)]
+
+
+def test_step_on_a_slice_of_a_pool_of_odd_states():
+    """States of 3 x 3 floats: the pool's second one starts at byte 36."""
+    from sorernn_b200 import linear_attention_step
+
+    x = inputs(2, 1, 1, 1, 3, 3, torch.float32, state=True, seed=6)
+    pool = torch.zeros(3, 1, 3, 3, device="cuda")
+    pool[1:] = x["h0"]
+    state = x["h0"].clone()
+    tokens = [x[n][:, 0] for n in ("q", "k", "v")]
+    want = linear_attention_step(*tokens, decays(1), state)
+    got = linear_attention_step(*tokens, decays(1), pool[1:])
+    assert torch.equal(got, want) and torch.equal(pool[1:], state) and not pool[0].any()
