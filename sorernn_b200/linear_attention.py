@@ -222,6 +222,25 @@ def chunk_linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s
     return o, (final if output_final_state else None)
 
 
+def _step(N, H, HV, K, V, scale, act_dtype, q, k, v, log_decay, state, slots, state_indices, out):
+    _call(q.device, _lib.lib().gdn_linear_attn_step, "gdn_linear_attn_step", N, H, HV, K, V, scale, act_dtype,
+          _at(q), _at(k), _at(v), _at(log_decay), _at(state), slots, _at(state_indices), _at(out))
+    return out
+
+
+class _Step(torch.autograd.Function):
+    """The step where autograd records: a backward through it says that there is none, instead of losing gradients."""
+
+    @staticmethod
+    def forward(ctx, args, *recorded):  # `out` in the tuple: an output, not an input, to autograd
+        return _step(*args)
+
+    @staticmethod
+    def backward(ctx, do):
+        raise RuntimeError("linear_attention_step has no backward (it updates its state in place): train through "
+                           "chunk_linear_attention")
+
+
 def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor,
                           scale: Optional[float] = None, state_indices: Optional[Tensor] = None,
                           out: Optional[Tensor] = None) -> Tensor:
@@ -231,7 +250,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     Without ``state_indices``, ``state`` is ``[N,HV,K,V]``. With ``state_indices`` (int32 ``[N]`` on the device, no two
     alike), ``state`` is a pool ``[slots,HV,K,V]`` and request n uses ``state[state_indices[n]]``; a negative index is
     an idle request (its output is zero, no state changes) and an index past the pool gives NaN and touches nothing.
-    Where V is a multiple of 4 the state's memory has to start on a 16-byte boundary.
+    Where V is a multiple of 4 the state's memory has to start on a 16-byte boundary. For decoding: there is no backward.
     """
     if not q.is_cuda:
         raise RuntimeError("sorernn_b200 runs on CUDA tensors only (no CPU fallback)")
@@ -264,7 +283,8 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     elif out.shape != v_shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {dtype} tensor {tuple(v_shape)} on {device}")
     scale = K ** -0.5 if scale is None else float(scale)
-    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-    _call(device, _lib.lib().gdn_linear_attn_step, "gdn_linear_attn_step", N, H, HV, K, V, scale, _DT[dtype],
-          _at(q), _at(k), _at(v), _at(log_decay), _at(state), s_shape[0], _at(state_indices), _at(out))
-    return out
+    args = (N, H, HV, K, V, scale, _DT[dtype], q.contiguous(), k.contiguous(), v.contiguous(), log_decay, state,
+            s_shape[0], state_indices, out)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        return _Step.apply(args, q, k, v, state)
+    return _step(*args)

@@ -89,3 +89,24 @@ def test_step_on_a_slice_of_a_pool_of_odd_states():
     want = linear_attention_step(*tokens, decays(1), state)
     got = linear_attention_step(*tokens, decays(1), pool[1:])
     assert torch.equal(got, want) and torch.equal(pool[1:], state) and not pool[0].any()
+
+
+def test_backward_through_a_step_is_an_error():
+    """Forward as under no_grad, an ``out`` tensor used twice too; a loss through it says that there is no backward."""
+    from sorernn_b200 import linear_attention_step
+
+    x = inputs(2, 1, 1, 2, 64, 64, torch.float32, state=True, seed=7)
+    tokens = [x[n][:, 0] for n in ("q", "k", "v")]
+    state = x["h0"].clone()
+    want = [linear_attention_step(*tokens, decays(2), state) for _ in range(2)]
+    for i in range(3):
+        got_state, out = x["h0"].clone(), torch.empty_like(want[0])
+        leaves = [t.detach().clone().requires_grad_(n == i) for n, t in enumerate(tokens)]
+        for w in want:
+            o = linear_attention_step(*leaves, decays(2), got_state, out=out)
+            assert o is out and torch.equal(o, w)
+            with pytest.raises(RuntimeError, match="no backward"):
+                o.sum().backward()
+        assert torch.equal(got_state, state)
+        with torch.no_grad():
+            assert not linear_attention_step(*leaves, decays(2), got_state).requires_grad
