@@ -19,6 +19,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from .gated_delta_rule import _DT
@@ -32,6 +33,13 @@ def _aligned(t: Optional[Tensor]) -> Optional[Tensor]:
     """``t`` (contiguous), or a copy where its memory starts off the library's 16-byte grid, as that of a slice may;
     autograd hands such slices over as gradients, of a concatenation for instance."""
     return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _refuse_tangents(name: str, *tensors: Optional[Tensor]) -> None:
+    """The kernels have no forward-mode derivative, and read the primal values alone."""
+    if getattr(forward_ad, "_current_level", -1) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _call(device: torch.device, fn, name: str, *args) -> None:
@@ -214,7 +222,9 @@ def chunk_linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s
     args = (q, k, v, log_decay, initial_state, cu_seqlens, scale, max_seqlen, output_final_state)
     if torch.compiler.is_compiling():
         o, final = linear_attn_fwd(*args)
-    elif torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+        return o, (final if output_final_state else None)
+    _refuse_tangents("chunk_linear_attention", q, k, v, initial_state)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                       initial_state is not None and initial_state.requires_grad):
         o, final = _LinearAttn.apply(*args)
     else:
@@ -285,6 +295,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     scale = K ** -0.5 if scale is None else float(scale)
     args = (N, H, HV, K, V, scale, _DT[dtype], q.contiguous(), k.contiguous(), v.contiguous(), log_decay, state,
             s_shape[0], state_indices, out)
+    _refuse_tangents("linear_attention_step", q, k, v, state)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         return _Step.apply(args, q, k, v, state)
     return _step(*args)

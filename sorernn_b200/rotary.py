@@ -17,7 +17,7 @@ from torch import Tensor
 
 from . import _lib
 from .gated_delta_rule import _DT
-from .linear_attention import _at, _call
+from .linear_attention import _at, _call, _refuse_tangents
 
 
 def rotary_table(max_positions: int, rotary_dim: int, theta: float = 10000.0,
@@ -166,6 +166,7 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, table
             float(eps))
     if torch.compiler.is_compiling():
         return qk_norm_rope_fwd(*args)
+    _refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or
                                     k_weight.requires_grad):
         return _QkNormRope.apply(*args)

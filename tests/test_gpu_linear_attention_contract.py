@@ -110,3 +110,24 @@ def test_backward_through_a_step_is_an_error():
         assert torch.equal(got_state, state)
         with torch.no_grad():
             assert not linear_attention_step(*leaves, decays(2), got_state).requires_grad
+
+
+def test_forward_mode_tangents_are_refused():
+    """There is no forward-mode derivative: an input that carries a tangent is refused, others pass within dual_level."""
+    import torch.autograd.forward_ad as fw
+
+    from sorernn_b200 import chunk_linear_attention, linear_attention_step, qk_norm_rope, rotary_table
+
+    x = inputs(1, 5, 2, 2, 64, 64, torch.float32, state=True, seed=8)
+    w, table, pos = torch.ones(64, device="cuda"), rotary_table(8, 32, device="cuda"), torch.arange(5, device="cuda")[None]
+    calls = [(["q", "k", "v", "h0"], lambda q, k, v, h0: chunk_linear_attention(q, k, v, decays(2), initial_state=h0)),
+             (["q", "k", "v", "h0"],
+              lambda q, k, v, h0: linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decays(2), h0)),
+             (["q", "k", "w"], lambda q, k, w: qk_norm_rope(q, k, w, w, table, pos))]
+    x["w"] = w
+    with fw.dual_level():
+        for names, call in calls:
+            call(*(x[n].clone() for n in names))
+            for m in names:
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*(fw.make_dual(x[n].clone(), torch.ones_like(x[n])) if n == m else x[n].clone() for n in names))
