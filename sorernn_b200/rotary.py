@@ -130,7 +130,7 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, table
     up to R/2) ``[len(sections),B,T]``: the first ``sections[0]`` pairs turn by axis 0, and so on. Pairs are
     ``(i, i + R/2)``, or ``(2i, 2i + 1)`` when ``interleaved``. A position outside the table makes its rotated features
     NaN. q and k may be strided views (features contiguous), such as slices of one projection's output. Gradients
-    reach q, k and the weights.
+    reach q, k and the weights; a table that requires one is refused.
     """
     if not q.is_cuda:
         raise RuntimeError("sorernn_b200 runs on CUDA tensors only (no CPU fallback)")
@@ -149,6 +149,8 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, table
     if len(t_shape) != 2 or table.dtype != torch.float32 or t_shape[1] % 2 or not 0 < t_shape[1] <= D:
         raise ValueError(f"table must be fp32 [P,R] with R even and at most {D}, got {table.dtype} "
                          f"{tuple(t_shape)}")
+    if table.requires_grad and torch.is_grad_enabled():
+        raise ValueError("table takes no gradient: the angles are a constant of the model")
     sections = [int(n) for n in sections] if sections else []
     if sections and (len(sections) > 4 or min(sections) < 0 or 2 * sum(sections) != t_shape[1]):
         raise ValueError(f"sections must be at most four counts adding up to R/2 = {t_shape[1] // 2}, got "

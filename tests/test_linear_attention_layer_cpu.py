@@ -60,3 +60,24 @@ def test_documents_past_the_table_are_refused():
             layer(x, **kw)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         layer(x[:, :16])
+
+
+def test_a_table_that_wants_gradients_is_refused(monkeypatch):
+    """The rotation gives its table no gradient; under no_grad there is none to lose."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from sorernn_b200 import _lib, qk_norm_rope
+
+    def called():
+        raise AssertionError("the library")
+
+    monkeypatch.setattr(_lib, "lib", called)
+    with FakeTensorMode():
+        q, w = torch.empty(1, 8, 2, 64, device="cuda"), torch.empty(64, device="cuda")
+        table = torch.empty(9, 32, device="cuda", requires_grad=True)
+        pos = torch.empty(1, 8, dtype=torch.int64, device="cuda")
+        with pytest.raises(ValueError, match="table takes no gradient"):
+            qk_norm_rope(q, q, w, w, table, pos)
+        with torch.no_grad(), pytest.raises(Exception) as e:
+            qk_norm_rope(q, q, w, w, table, pos)
+        assert "no gradient" not in str(e.value)
