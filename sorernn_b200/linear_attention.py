@@ -235,6 +235,7 @@ def chunk_linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, s
 def _step(N, H, HV, K, V, scale, act_dtype, q, k, v, log_decay, state, slots, state_indices, out):
     _call(q.device, _lib.lib().gdn_linear_attn_step, "gdn_linear_attn_step", N, H, HV, K, V, scale, act_dtype,
           _at(q), _at(k), _at(v), _at(log_decay), _at(state), slots, _at(state_indices), _at(out))
+    torch.autograd.graph.increment_version((state, out))  # written in place: autograd may have saved them
     return out
 
 

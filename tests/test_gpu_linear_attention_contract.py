@@ -131,3 +131,19 @@ def test_forward_mode_tangents_are_refused():
             for m in names:
                 with pytest.raises(NotImplementedError, match="forward-mode"):
                     call(*(fw.make_dual(x[n].clone(), torch.ones_like(x[n])) if n == m else x[n].clone() for n in names))
+
+
+def test_a_step_on_a_state_that_autograd_saved_is_noticed():
+    """A prefill from a state, then a step on that state in place: the prefill's backward needs the old values."""
+    from sorernn_b200 import chunk_linear_attention, linear_attention_step
+
+    x = inputs(1, 5, 1, 1, 64, 64, torch.float32, state=True, seed=9)
+    q = x["q"].clone().requires_grad_(True)
+    o, _ = chunk_linear_attention(q, x["k"], x["v"], decays(1), initial_state=x["h0"])
+    with torch.no_grad():
+        linear_attention_step(x["q"][:, 0], x["k"][:, 0], x["v"][:, 0], decays(1), x["h0"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.backward(x["do"])
+    with torch.inference_mode():
+        state = x["h0"].clone()
+        linear_attention_step(x["q"][:, 0], x["k"][:, 0], x["v"][:, 0], decays(1), state)
