@@ -88,7 +88,8 @@ static ScanPlan plan(const gdn_linear_attn_problem* p, int64_t DB, int64_t DC, i
     s.items = item_count(p->B, p->T, p->N, p->cu_seqlens != nullptr, per);
     s.cut = p->T > per;
     s.end_in_join = s.tc && !p->cu_seqlens;
-    s.local_bytes = s.cut ? round256((size_t)s.items * p->HV * DB * DC * sizeof(float)) : 0;
+    const int64_t states = state_count(p->T, s.items, p->cu_seqlens != nullptr, per);
+    s.local_bytes = s.cut ? round256((size_t)states * p->HV * DB * DC * sizeof(float)) : 0;
     return s;
 }
 
@@ -128,7 +129,7 @@ static int scan(const gdn_linear_attn_problem* p, Scans b, void* local, cudaStre
     return launch(0);
 }
 
-// Joins the pieces' own end states along each sequence, in place: local[piece] becomes the state that reaches the piece
+// Joins the pieces' own end states along each sequence, in place: a piece's becomes the state that reaches the next one
 // (X <- a^len X + local in scan order, X from x0). One thread per 4 elements of a (sequence, value head)'s state; the
 // loads of the pieces do not depend on one another, so a chain of P pieces costs about one memory latency for every
 // four of them (5 us for 16 heads of a 65,536-token sequence), where each CTA of the scan joining for itself cost two
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(256) linear_attn_join_kernel(const __grid_cons
     const int64_t n = blockIdx.x / a.HV, per = (int64_t)a.chunk * a.piece_chunks;
     const int64_t len = a.cu ? a.cu[n + 1] - a.cu[n] : a.T;
     const int pieces = len > 0 ? (int)((len + per - 1) / per) : 1;
-    if (pieces == 1 && !a.x0 && !a.end_in_join) return;  // nothing to join, and nothing is read
+    if (pieces == 1 && !a.end_in_join) return;  // nothing to join
     int64_t item0 = n * pieces;
     if (a.cu) {
         int64_t part = 0;  // pieces of the sequences before this one
@@ -172,16 +173,16 @@ __global__ void __launch_bounds__(256) linear_attn_join_kernel(const __grid_cons
     const int last = pieces - 1;
     const float f_last = expf(g * (float)(len - last * per));
     const int own = a.end_in_join ? pieces : last;  // pieces with a state of their own, in scan order
-    float* const l = a.local + e + (item0 * a.HV + hv) * (int64_t)size;
+    float* const l = a.local + e + (state_slot(a, n, item0, 0) * a.HV + hv) * (int64_t)size;
     const int64_t step = (int64_t)a.HV * size;
     const bool vec = size % 4 == 0;
-    for (int i0 = 0; i0 < pieces; i0 += 4) {
+    for (int i0 = 0; i0 < own; i0 += 4) {
         float y[4][4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int i = i0 + u;
             if (i >= own) continue;
-            const float* const src = l + (a.reverse ? last - i : i) * step;
+            const float* const src = l + i * step;
             if (vec) *reinterpret_cast<float4*>(y[u]) = *reinterpret_cast<const float4*>(src);
             else
                 for (int k = 0; k < valid; ++k) y[u][k] = src[k];
@@ -189,17 +190,15 @@ __global__ void __launch_bounds__(256) linear_attn_join_kernel(const __grid_cons
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int i = i0 + u;
-            if (i > last) continue;
-            float* const dst = l + (a.reverse ? last - i : i) * step;
-            if (i == 0 && !a.x0) {  // nothing reaches it, and nothing is read
+            if (i >= own) continue;
+            const float fi = i == (a.reverse ? 0 : last) ? f_last : f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) X[k] = fmaf(fi, X[k], y[u][k]);
+            float* const dst = l + i * step;
+            if (i == last) {  // no piece follows
             } else if (vec) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<float4*>(X);
             else
                 for (int k = 0; k < valid; ++k) dst[k] = X[k];
-            if (i < own) {
-                const float fi = i == (a.reverse ? 0 : last) ? f_last : f;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) X[k] = fmaf(fi, X[k], y[u][k]);
-            }
         }
     }
     if (a.end_in_join) {

@@ -103,7 +103,6 @@ __global__ void __launch_bounds__(sk::NTHR) linear_attn_fp32_kernel(const __grid
     const int64_t len = eos - bos, chunks = (len + C - 1) / C;
     const int64_t pieces = chunks > 0 ? (chunks + a.piece_chunks - 1) / a.piece_chunks : 1;
     const bool last = a.reverse ? p == 0 : p == pieces - 1;   // the piece that leaves the sequence
-    const bool first = a.reverse ? p == pieces - 1 : p == 0;  // in scan order: only x0 reaches it
     if (!OUT && last) return;
     const int64_t ch_lo = p * a.piece_chunks;
     const int64_t ch_hi = ch_lo + a.piece_chunks < chunks ? ch_lo + a.piece_chunks : chunks;
@@ -156,14 +155,16 @@ __global__ void __launch_bounds__(sk::NTHR) linear_attn_fp32_kernel(const __grid
     float X[NT][4];
     const int64_t xbase = (n * a.HV + hv) * (int64_t)a.DB * a.DC;
     auto x_at = [&](int r, int c) { return xbase + (a.transposed ? (int64_t)c * a.DB + r : (int64_t)r * a.DC + c); };
-    const float* const from = !OUT || (first && !a.x0) ? nullptr
-                              : a.local ? a.local + (item * a.HV + hv) * (int64_t)a.DB * a.DC : a.x0;
+    const int64_t order = a.reverse ? pieces - 1 - p : p;  // in scan order; only x0 reaches the first
+    const int64_t slot = state_slot(a, n, item - p, OUT ? order - 1 : order);
+    const bool joined = OUT && order > 0;
+    const float* const from = !OUT ? nullptr : joined ? a.local + (slot * a.HV + hv) * (int64_t)a.DB * a.DC : a.x0;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int r = xr + gr + 8 * (e >> 1), x = xc + 8 * i + 2 * tq + (e & 1);
-            X[i][e] = from && r < a.DB && x < cw ? from[a.local ? (int64_t)r * a.DC + x : x_at(r, x)] : 0.f;
+            X[i][e] = from && r < a.DB && x < cw ? from[joined ? (int64_t)r * a.DC + x : x_at(r, x)] : 0.f;
         }
     // outputs: 16 rows from orw, OT tiles of 8 columns from oc; P: 16 rows from orw, 8 columns from 8 (warp / 2)
     constexpr int OT = CW / 32;
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(sk::NTHR) linear_attn_fp32_kernel(const __grid
             const int r = xr + gr + 8 * (e >> 1), x = xc + 8 * i + 2 * tq + (e & 1);
             if (r < a.DB && x < cw) {
                 if (OUT) dst[x_at(r, x)] = X[i][e];
-                else dst[(item * a.HV + hv) * (int64_t)a.DB * a.DC + (int64_t)r * a.DC + x] = X[i][e];
+                else dst[(slot * a.HV + hv) * (int64_t)a.DB * a.DC + (int64_t)r * a.DC + x] = X[i][e];
             }
         }
 }

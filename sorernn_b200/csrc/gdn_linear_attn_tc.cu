@@ -62,12 +62,13 @@ constexpr uint32_t T_P = 0, T_U = 128, T_OI = 256, T_OA = 384, T_COLS = 512;  //
 constexpr uint32_t BLK = C * 128;  // bytes of a 64-feature block of a tile
 
 // What a CTA works on. Kept in shared memory, so that each role loads what it needs into its own registers.
-struct Info {
+struct alignas(16) Info {
     int n, bos, eos;          // sequence, its first token, the token past its end
     int n_precise;            // a chunk's split takes a third term where fewer tokens than this follow in scan order
     int tok_first, tok_step;  // first token of the first chunk in scan order; from chunk to chunk
     int nch, n_u;             // chunks; chunks whose U is formed
     int last, has_x;          // the piece that leaves the sequence; a state comes in
+    int slot;                 // place in `local` of that state (-1: it is x0's), or (without outputs) of this piece's own
     uint32_t tm;              // tensor memory
     int failed;               // a warp of the outputs' role gave up
 };
@@ -95,6 +96,7 @@ struct Smem {
     static constexpr uint32_t INFO = BAR + 20 * 8;  // NBAR barriers
     static constexpr uint32_t RED = INFO + sizeof(Info);
     static constexpr uint32_t END = RED + (NTHR / 32 + 3) * 8;
+    static_assert(TAB % 16 == 0 && BAR % 8 == 0 && INFO % 16 == 0 && RED % 8 == 0, "alignment of the blocks' parts");
     // more than half of an SM's shared memory, so that one CTA holds the SM's tensor memory
     static constexpr uint32_t BYTES = (END > 120 * 1024 ? END : 120 * 1024) + 1024;
 };
@@ -282,7 +284,9 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
             info->n_u = !OUT || (last && a.x1) ? nch : nch - 1;  // the last chunk's only if its end state is wanted
             info->last = last;
             info->failed = 0;
-            info->has_x = OUT && (a.x0 || (a.local && (a.reverse ? p < pieces - 1 : p > 0)));
+            const int order = a.reverse ? pieces - 1 - p : p;  // in scan order; only x0 reaches the first
+            info->has_x = OUT && (order > 0 || a.x0);
+            info->slot = OUT && order == 0 ? -1 : (int)state_slot(a, n, item - p, order - (OUT ? 1 : 0));
         }
     }
     if (tid == 16 * 32) {
@@ -503,10 +507,11 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
         float2 x[XC / 2];
         const int64_t xrow = ((int64_t)info->n * a.HV + hv) * (int64_t)DB * DC + (a.transposed ? row * DB : row);
         const int xs = a.transposed ? 1 : DC;  // x0, x1: column j at xrow + j xs
-        const int64_t lrow = ((int64_t)(cta / a.HV) * a.HV + hv) * DB * DC + x0c * DC + row;  // in `local`
+        const int64_t lrow = ((int64_t)info->slot * a.HV + hv) * DB * DC + x0c * DC + row;  // in `local`
         const bool from = OUT && info->has_x && live;
-        const float* const src = a.local ? a.local + lrow : a.x0 + xrow;
-        const int ss = a.local ? DC : xs;
+        const bool given = info->slot < 0;
+        const float* const src = given ? a.x0 + xrow : a.local + lrow;
+        const int ss = given ? xs : DC;
 #pragma unroll
         for (int j = 0; j < XC; j += 2)
             x[j / 2] = from ? make_float2(src[j * ss], src[(j + 1) * ss]) : make_float2(0.f, 0.f);

@@ -19,8 +19,9 @@
 // Chunks are counted from a sequence's first token in both directions; its last chunk may be partial. A sequence is
 // cut into pieces of `piece_chunks` chunks that run side by side: with more than one piece, a first launch
 // (states_only) leaves each piece's own end state (from zero) in `local`, a second joins them along the sequence, so that
-// `local` holds the state that reaches each piece, and the third runs the pieces from there. The end state comes from the
-// third launch, or (end_in_join) from the second.
+// `local` holds the state that reaches the next piece, and the third runs the pieces from there, the first one from x0. The
+// end state comes from the third launch, or (end_in_join) from the second. Packed sequences keep no state of their last
+// piece in scan order, so that the many of one piece take no memory.
 #pragma once
 #include "common.cuh"
 #include "kernels.h"
@@ -34,7 +35,7 @@ struct ScanArgs {
     const float* log_decay;   // [HV]
     const float* x0;          // incoming state [N, HV, DK, DV], or NULL
     float* x1;                // outgoing state [N, HV, DK, DV], or NULL
-    float* local;             // the pieces' states [items, HV, DB, DC], or NULL (one piece per sequence)
+    float* local;             // the pieces' states [state_count(), HV, DB, DC], or NULL (one piece per sequence)
     const int64_t* cu;
     int64_t T, N, items;      // items: (sequence, piece) pairs, with cu an upper bound
     int HV;
@@ -122,6 +123,14 @@ __device__ __forceinline__ bool locate(const ScanArgs& a, int64_t item, int64_t*
     }
     return false;
 }
+
+// The place in `local` of piece i's own end state, and after the join of the state that reaches piece i + 1; i counts the
+// pieces of sequence n in scan order, `first` is the sequence's first item.
+__device__ __forceinline__ int64_t state_slot(const ScanArgs& a, int64_t n, int64_t first, int64_t i) {
+    return first - (a.cu ? n : 0) + i;
+}
+// Places in `local`: sequences of len tokens have ceil(len / per) pieces, packed ones keep (len - 1) / per states.
+inline int64_t state_count(int64_t T, int64_t items, bool varlen, int64_t per) { return varlen ? T / per : items; }
 
 // Pieces per work list: exact for batches, an upper bound for packed sequences.
 inline int64_t item_count(int64_t B, int64_t T, int64_t N, bool varlen, int64_t per) {

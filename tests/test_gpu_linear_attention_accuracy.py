@@ -10,12 +10,14 @@ has none left), in units of RMS(ref). Bars, from the arithmetic:
     grows by sqrt(2), and five and a half standard deviations off (a million values): 5e-5; its fp32 sums add as much
     again: 2e-4 with a factor of two to spare.
 """
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
-from helpers import PARITY_LOG, CURRENT_TEST, rms
-from test_gpu_linear_attention import decays, inputs, oracle
+from helpers import CURRENT_TEST, PARITY_LOG, assert_rms_close, rms, to_np
+from test_gpu_linear_attention import FP32_TOL, decays, inputs, oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +71,34 @@ def test_tensor_memory_kernel_whole_sequences(K, V, decay):
 def test_tensor_memory_kernel_cut_sequences(K, V, T):
     """Pieces side by side, heads that never decay and heads that decay at once: the state enters every output."""
     run(2, T, 5, 5, K, V, torch.bfloat16, "edges", TC_TOL, seed=6)
+
+
+@pytest.mark.parametrize("known", [True, False])  # the lengths, on the host
+@pytest.mark.parametrize("dtype,tol", [(torch.bfloat16, TC_TOL), (torch.float32, None)])
+@pytest.mark.parametrize("H,HV", [(2, 2), (1, 2)])
+def test_packed_documents_cut_into_pieces(H, HV, dtype, tol, known):
+    """Documents of many pieces among ones of a single piece and empty ones, with and without states, K = V = 128: the
+    backward's three scans of a cut packed window in one launch. States and fp32 outputs to 5e-5 of RMS, as elsewhere."""
+    from sorernn_b200 import _lib, chunk_linear_attention
+
+    cu = [0, 0, 1, 2, 130, 1400, 1401, 1401, 1500, 3100, 3101, 3200]
+    N, T = len(cu) - 1, cu[-1]
+    p = _lib.LinearAttnProblem(1, T, HV, HV, 128, 128, N, 16, 1600 if known else 0, 0.1,
+                               _lib.BF16 if dtype == torch.bfloat16 else _lib.FP32)
+    assert _lib.lib().gdn_linear_attn_bwd_workspace_size(ctypes.byref(p)) > 0  # cut
+    cu_t = torch.tensor(cu, device="cuda")
+    for state in (False, True):
+        x = inputs(1, T, H, HV, 128, 128, dtype, N, state, 13)
+        ld = decays(HV, "-0.01")
+        leaves = [x[n].requires_grad_(True) for n in ("q", "k", "v") + (("h0",) if state else ())]
+        o, ht = chunk_linear_attention(x["q"], x["k"], x["v"], ld, initial_state=x["h0"], output_final_state=True,
+                                       cu_seqlens=cu_t, cu_seqlens_cpu=cu_t.cpu() if known else None)
+        grads = torch.autograd.grad((o, ht) if state else (o,), leaves, (x["do"], x["dht"]) if state else (x["do"],))
+        ref = oracle(x["q"], x["k"], x["v"], ld, 128 ** -0.5, cu, x["h0"], x["do"], x["dht"])
+        for n, y in zip(("o", "dq", "dk", "dv", "dh0", "ht"), (o, *grads, *(() if state else (None,)), ht)):
+            if y is None:
+                continue
+            if y.dtype == torch.float32:
+                assert_rms_close(to_np(y), ref[n].cpu().numpy(), FP32_TOL, "lin packed cut " + n)
+            else:
+                within("lin packed cut " + n, y, ref[n], tol)
