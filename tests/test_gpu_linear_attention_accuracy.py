@@ -9,6 +9,8 @@ has none left), in units of RMS(ref). Bars, from the arithmetic:
     the sum's own RMS. An element may be of a head whose RMS is 1.6 times that of all heads, late in a sequence whose RMS
     grows by sqrt(2), and five and a half standard deviations off (a million values): 5e-5; its fp32 sums add as much
     again: 2e-4 with a factor of two to spare.
+  * the other kernel (fp16, and bf16 of other head sizes) is good to fp32: FP32_TOL, the bar of fp32 activations, 5e-5. The
+    products in one tf32 term would leave 2^-11, ten times that.
 """
 import ctypes
 
@@ -102,3 +104,12 @@ def test_packed_documents_cut_into_pieces(H, HV, dtype, tol, known):
                 assert_rms_close(to_np(y), ref[n].cpu().numpy(), FP32_TOL, "lin packed cut " + n)
             else:
                 within("lin packed cut " + n, y, ref[n], tol)
+
+
+@pytest.mark.parametrize("dtype,K,V", [(torch.float16, 128, 128), (torch.float16, 64, 64), (torch.float16, 20, 33),
+                                       (torch.bfloat16, 96, 128), (torch.bfloat16, 20, 33), (torch.bfloat16, 128, 7)])
+@pytest.mark.parametrize("decay", ["slopes", "edges"])
+def test_fp32_kernel(dtype, K, V, decay):
+    """Whole (16 sequences) and cut (one long one)."""
+    run(16, 100, 5, 10, K, V, dtype, decay, FP32_TOL, seed=14)
+    run(1, 1500, 2, 2, K, V, dtype, decay, FP32_TOL, seed=15)

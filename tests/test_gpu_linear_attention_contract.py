@@ -147,3 +147,58 @@ def test_a_step_on_a_state_that_autograd_saved_is_noticed():
     with torch.inference_mode():
         state = x["h0"].clone()
         linear_attention_step(x["q"][:, 0], x["k"][:, 0], x["v"][:, 0], decays(1), state)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_cuda_graph_capture(dtype):
+    """Forward and backward (a cut sequence), a decode step and the norm with rotation, captured once and replayed on new
+    inputs: the same bits as the calls outside."""
+    from sorernn_b200 import chunk_linear_attention, linear_attention_step, qk_norm_rope, rotary_table
+
+    T = 1500
+    x = inputs(1, T, 2, 4, 128, 128, dtype, state=True, seed=10)
+    ld, w = decays(4), torch.ones(128, device="cuda", requires_grad=True)
+    table, pos = rotary_table(T, 32, device="cuda"), torch.arange(T, device="cuda")[None]
+    leaves = [x[n].requires_grad_(True) for n in ("q", "k", "v", "h0")]
+    token, state = [x[n].detach()[:, 7].clone() for n in ("q", "k", "v")], x["h0"].detach().clone()
+
+    def work():
+        q, k = qk_norm_rope(x["q"], x["k"], w, w, table, pos)
+        o, ht = chunk_linear_attention(q, k, x["v"], ld, initial_state=x["h0"], output_final_state=True)
+        grads = torch.autograd.grad((o, ht), leaves + [w], (x["do"], x["dht"]))
+        with torch.no_grad():
+            return [o, ht, *grads, linear_attention_step(*token, ld, state)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    fresh = inputs(1, T, 2, 4, 128, 128, dtype, state=True, seed=11)
+    with torch.no_grad():
+        for n, t in fresh.items():
+            x[n].copy_(t)
+        start = torch.randn_like(state)
+        state.copy_(start)
+        graph.replay()
+        got, got_state = [t.clone() for t in out], state.clone()
+        state.copy_(start)
+    want = work()
+    assert torch.equal(got_state, state)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs in one process")
+def test_tensors_on_another_device_than_the_current_one():
+    from sorernn_b200 import chunk_linear_attention
+
+    x = inputs(1, 300, 2, 2, 128, 128, torch.bfloat16, seed=12)
+    ld = decays(2)
+    want = chunk_linear_attention(x["q"], x["k"], x["v"], ld, output_final_state=True)
+    got = chunk_linear_attention(*(x[n].to("cuda:1") for n in ("q", "k", "v")), ld.to("cuda:1"), output_final_state=True)
+    for a, b in zip(want, got):
+        assert b.device.index == 1 and torch.equal(a.cpu(), b.cpu())
