@@ -9,7 +9,7 @@
 namespace gdn {
 namespace linattn {
 
-constexpr int kSimtChunk = 32, kTcChunk = 128;
+constexpr int kFp32Chunk = 32, kTcChunk = 128;
 
 static bool dtype_ok(int32_t d) { return d == GDN_BF16 || d == GDN_FP16 || d == GDN_FP32; }
 static size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -78,7 +78,7 @@ struct ScanPlan {
 static ScanPlan plan(const gdn_linear_attn_problem* p, int64_t DB, int64_t DC, int n_scans) {
     ScanPlan s{};
     s.tc = scan_tc_supported(DB, DC, p->act_dtype);
-    s.chunk = s.tc ? kTcChunk : kSimtChunk;
+    s.chunk = s.tc ? kTcChunk : kFp32Chunk;
     const int64_t sms = device_sm_count();
     // measured: a chunk 4.7 us (128 tokens, tensor cores), start-up 5.7, states-only chunk 2.1, the two more launches 7
     const PieceCost cost = s.tc ? PieceCost{sms, 1.2, 0.45, 1.5, 0.1}
@@ -114,7 +114,7 @@ static int scan(const gdn_linear_attn_problem* p, Scans b, void* local, cudaStre
     }
     auto launch = [&](int states_only) {
         for (int i = 0; i < b.n; ++i) b.s[i].states_only = states_only;
-        return sp.tc ? scan_tc(b, p->B * p->T, s) : scan_simt(b, p->act_dtype, s);
+        return sp.tc ? scan_tc(b, p->B * p->T, s) : scan_fp32(b, p->act_dtype, s);
     };
     if (sp.cut) {
         int st = launch(1);

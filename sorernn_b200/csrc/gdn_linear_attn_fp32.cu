@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(sk::NTHR) linear_attn_fp32_kernel(const __grid
 }
 
 template <typename TA, int DB, int CW, bool OUT>
-static int launch_simt(const Scans& b, cudaStream_t s) {
+static int launch_fp32(const Scans& b, cudaStream_t s) {
     constexpr int smem = (int)sk::Smem<TA, DB, CW>::BYTES;
     const void* k = (const void*)linear_attn_fp32_kernel<TA, DB, CW, OUT>;
     if (smem_optin(k, smem) != cudaSuccess) return GDN_ERR_LAUNCH;
@@ -316,22 +316,22 @@ static int launch_simt(const Scans& b, cudaStream_t s) {
 }
 
 template <typename TA, int DB, int CW>
-static int simt_mode(const Scans& b, cudaStream_t s) {
-    return b.s[0].states_only ? launch_simt<TA, DB, CW, false>(b, s) : launch_simt<TA, DB, CW, true>(b, s);
+static int fp32_mode(const Scans& b, cudaStream_t s) {
+    return b.s[0].states_only ? launch_fp32<TA, DB, CW, false>(b, s) : launch_fp32<TA, DB, CW, true>(b, s);
 }
 
 template <typename TA>
-static int simt_typed(const Scans& b, cudaStream_t s) {
-    if (b.s[0].DB <= 64) return b.s[0].DC <= 64 ? simt_mode<TA, 64, 64>(b, s) : simt_mode<TA, 64, 128>(b, s);
-    return b.s[0].DC <= 64 ? simt_mode<TA, 128, 64>(b, s) : simt_mode<TA, 128, 128>(b, s);
+static int fp32_typed(const Scans& b, cudaStream_t s) {
+    if (b.s[0].DB <= 64) return b.s[0].DC <= 64 ? fp32_mode<TA, 64, 64>(b, s) : fp32_mode<TA, 64, 128>(b, s);
+    return b.s[0].DC <= 64 ? fp32_mode<TA, 128, 64>(b, s) : fp32_mode<TA, 128, 128>(b, s);
 }
 
-int scan_simt(const Scans& b, int act_dtype, cudaStream_t s) {
+int scan_fp32(const Scans& b, int act_dtype, cudaStream_t s) {
     if (b.s[0].items * b.s[0].HV * b.n > 0x7fffffff) return GDN_ERR_SHAPE;
     switch (act_dtype) {
-        case GDN_BF16: return simt_typed<__nv_bfloat16>(b, s);
-        case GDN_FP16: return simt_typed<__half>(b, s);
-        case GDN_FP32: return simt_typed<float>(b, s);
+        case GDN_BF16: return fp32_typed<__nv_bfloat16>(b, s);
+        case GDN_FP16: return fp32_typed<__half>(b, s);
+        case GDN_FP32: return fp32_typed<float>(b, s);
         default: return GDN_ERR_DTYPE;
     }
 }

@@ -25,7 +25,7 @@
 //   warp 17      issues the loads (single buffers; L2 prefetch two chunks ahead)
 // 8 x 4,096 tokens x 16 heads, DB = DC = 128: a scan takes 149 us, 4.7 us a chunk, 0.55 of a copy's rate over the four
 // tensors that it reads and writes; bound by the hand-overs between the roles and the products' shared-memory reads. The
-// fp32-accuracy kernel (gdn_linear_attn_simt.cu) takes 903 us (64 features: 417 against 90; one chunk of 16 heads: 36
+// fp32-accuracy kernel (gdn_linear_attn_fp32.cu) takes 903 us (64 features: 417 against 90; one chunk of 16 heads: 36
 // against 25 with the call), so bf16 runs here at every size that this one supports. The states-only form runs the split,
 // its product and the accumulator in two buffers each and loads B a whole chunk ahead: 2.1 us a chunk (159 us for the pieces
 // of 65,536 tokens x 16 heads with one buffer and half a chunk ahead, 118 so). What decided the layout with outputs,
@@ -223,21 +223,6 @@ __device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 
 __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
 __device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// two fp32 operations in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t&>(d))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(d))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-    return d;
-}
 template <int N> __device__ __forceinline__ void set_regs() {
     if constexpr (N > 96) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
     if constexpr (N < 96) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));

@@ -138,7 +138,7 @@ inline int64_t item_count(int64_t B, int64_t T, int64_t N, bool varlen, int64_t 
 }
 
 // All scans of a batch have the same sizes (DB, DC, HV, items, chunking) and the same states_only.
-int scan_simt(const Scans& b, int act_dtype, cudaStream_t s);
+int scan_fp32(const Scans& b, int act_dtype, cudaStream_t s);
 bool scan_tc_supported(int64_t DB, int64_t DC, int act_dtype);
 int scan_tc(const Scans& b, int64_t tokens, cudaStream_t s);
 
