@@ -70,8 +70,8 @@ struct ScanPlan {
     int64_t items;
     bool cut;
     // The end state from the join: the tensor-memory kernel with outputs is a fifth slower where it has to keep a state to
-    // fp32 (1x65536x16: 284 us against 222), and the last pieces of equal sequences fit the states' launch without another
-    // wave. Packed documents, many of them of one piece, would run their states for nothing else.
+    // fp32 (1x65536x16: the whole call 473 us against 412), and the last pieces of equal sequences fit the states' launch
+    // without another wave. Packed documents, many of them of one piece, would run their states for nothing else.
     bool end_in_join;
     size_t local_bytes;
 };
@@ -80,8 +80,14 @@ static ScanPlan plan(const gdn_linear_attn_problem* p, int64_t DB, int64_t DC, i
     s.tc = scan_tc_supported(DB, DC, p->act_dtype);
     s.chunk = s.tc ? kTcChunk : kFp32Chunk;
     const int64_t sms = device_sm_count();
-    // measured: a chunk 4.7 us (128 tokens, tensor cores), start-up 5.7, states-only chunk 2.1, the two more launches 7
-    const PieceCost cost = s.tc ? PieceCost{sms, 1.2, 0.45, 1.5, 0.1}
+    // Measured, on tensor memory (128 tokens): a chunk 4.7 us, its start-up 5.7 (1.2 chunks), a states-only chunk 1.8 to
+    // 2.1 (0.4), the two more launches 7 (1.5), a piece more to join 0.15. In tf32 (32 tokens): a chunk 9.7 us in fp32 and
+    // 7.1 in fp16 (64 features, two CTAs an SM: 6.2), start-up 0.7 to 0.9 chunks, states-only 0.43, the launches 0.7 to 1.1.
+    // The model charges the cut somewhat more than that, for packed windows, where it knows the lengths no better than by
+    // the longest: with the measured values single batches of 70 drawn ones gain (2x552 of 4 heads 68 us to 58, all
+    // others within 3 %), but forward and backward of 4,295 tokens in 7 documents of 17 bf16 heads go from 166 to 192 us, of
+    // 2,969 in 18 documents of 20 fp32 heads from 478 to 590.
+    const PieceCost cost = s.tc ? PieceCost{sms, 1.5, 0.55, 1.8, 0.1}
                                 : PieceCost{sms * (DB <= 64 && DC <= 64 ? 2 : 1), 0.5, 0.6, 1.8, 0.1};
     s.piece_chunks = choose_piece_chunks(p, s.chunk, p->HV * n_scans, cost);
     const int64_t per = (int64_t)s.chunk * s.piece_chunks;

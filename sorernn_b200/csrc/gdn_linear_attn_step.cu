@@ -4,8 +4,9 @@
 // stream at the memory's copy speed. A CTA takes one (request, value head) and a slice of the state's columns
 // (columns are independent: no sums cross CTAs). Its threads hold ROWS rows of 4 columns each, all loads issued
 // before the first use. Slices are 64 columns: with the whole 128 a CTA's registers leave two on an SM, which then
-// load and store in phase (256 requests x 16 heads: 121 us against 90, 0.92 of the copy rate); 32 where the states
-// are too few to fill the SMs (16 of them: 2.5 us against 2.7).
+// load and store in phase (256 requests x 16 heads: 121 us against 90, 0.92 of the copy rate); 32 where there is an
+// SM for every such slice (16 states of 128 columns: 2.4 us against 2.7, 32: 2.5 against 2.7, but 64: 2.9 against 2.8 and
+// 128: 3.9 against 3.5).
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.h"
@@ -123,7 +124,7 @@ extern "C" int gdn_linear_attn_step(int64_t N, int64_t H, int64_t HV, int64_t DK
     a.n_slots = n_slots;
     a.H = (int)H; a.HV = (int)HV; a.DK = (int)DK; a.DV = (int)DV; a.scale = scale;
     cudaStream_t s = (cudaStream_t)stream;
-    const bool few = N * HV * 2 < 2 * (int64_t)device_sm_count();  // fewer than two 64-column CTAs an SM
+    const bool few = N * HV * ((DV + 31) / 32) <= device_sm_count();  // an SM for every 32-column slice
     GDN_DISPATCH_DTYPE(act_dtype, TA, {
         if (DV % 4) launch<TA, 1, 32>(a, N, s);
         else if (few) launch<TA, 4, 32>(a, N, s);
