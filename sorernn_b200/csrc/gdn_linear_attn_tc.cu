@@ -490,16 +490,24 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
         const bool live = row < DC;
         const uint32_t lb = (uint32_t)(row & 96) << 16;
         float2 x[XC / 2];
-        const int64_t xrow = ((int64_t)info->n * a.HV + hv) * (int64_t)DB * DC + (a.transposed ? row * DB : row);
-        const int xs = a.transposed ? 1 : DC;  // x0, x1: column j at xrow + j xs
+        const int64_t xrow = ((int64_t)info->n * a.HV + hv) * (int64_t)DB * DC;               // of x0 and x1
         const int64_t lrow = ((int64_t)info->slot * a.HV + hv) * DB * DC + x0c * DC + row;  // in `local`
         const bool from = OUT && info->has_x && live;
         const bool given = info->slot < 0;
-        const float* const src = given ? a.x0 + xrow : a.local + lrow;
-        const int ss = given ? xs : DC;
+        const float* const src = given ? a.x0 + xrow + (a.transposed ? row * DB : row) : a.local + lrow;
 #pragma unroll
-        for (int j = 0; j < XC; j += 2)
-            x[j / 2] = from ? make_float2(src[j * ss], src[(j + 1) * ss]) : make_float2(0.f, 0.f);
+        for (int j = 0; j < XC / 2; ++j) x[j] = make_float2(0.f, 0.f);
+        if (from && given && a.transposed) {  // a thread's row is contiguous: by 16 bytes
+#pragma unroll
+            for (int j = 0; j < XC; j += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(src + j);
+                x[j / 2] = make_float2(y.x, y.y);
+                x[j / 2 + 1] = make_float2(y.z, y.w);
+            }
+        } else if (from) {  // column by column, a warp's threads side by side
+#pragma unroll
+            for (int j = 0; j < XC; j += 2) x[j / 2] = make_float2(src[j * DC], src[(j + 1) * DC]);
+        }
         auto write_x = [&](int c) {  // X^T: row = feature of C, DB along the row
 #pragma unroll
             for (int j = 0; j < DB; j += 8) {
@@ -557,12 +565,11 @@ __global__ void __launch_bounds__(tk::NTHR, 1) linear_attn_tc_kernel(const __gri
         float* dst = OUT ? (info->last ? a.x1 : nullptr) : a.local;
         if (gave_up()) dst = nullptr;
         if (dst && live) {
-            dst += OUT ? xrow : lrow;
-            const int ds = OUT ? xs : DC;
+            dst += OUT ? xrow + row : lrow;  // x1 is never transposed
 #pragma unroll
             for (int j = 0; j < XC; j += 2) {
-                dst[j * ds] = x[j / 2].x;
-                dst[(j + 1) * ds] = x[j / 2].y;
+                dst[j * DC] = x[j / 2].x;
+                dst[(j + 1) * DC] = x[j / 2].y;
             }
         }
     } else if (warp >= 8) {

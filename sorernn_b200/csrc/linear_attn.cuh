@@ -43,7 +43,7 @@ struct ScanArgs {
     int DB, DC;               // row sizes: of A and B, of C and out
     int piece_chunks;
     int chunk;                // tokens per chunk
-    int reverse, transposed;  // transposed: x0, x1 are stored [DC, DB]
+    int reverse, transposed;  // transposed: x0 is stored [DC, DB] (such a scan has no x1)
     int states_only;
     int out_fp32;
     int precise;              // the state itself is wanted (x1): keep it to fp32 accuracy
