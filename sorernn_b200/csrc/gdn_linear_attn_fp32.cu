@@ -13,8 +13,8 @@
 // X is copied to shared memory once a chunk for the read-out. The next chunk's rows come in by asynchronous copies (two
 // stages, in the activations' type) while this one is worked on; rows that are not whole 16-byte vectors are loaded by
 // element. Row strides keep the fragments' loads free of bank conflicts, but for B's transposed ones (two-way). Bound by
-// the instructions that split and load the fragments: 4 x 1,024 tokens x 16 heads of 128, forward and backward, 878 us in
-// fp32 and 640 us in fp16 (20 and 27 TFLOP/s of what the recurrences need). As fp32 FMAs the same tiling took 1,205
+// the instructions that split and load the fragments: 4 x 1,024 tokens x 16 heads of 128, forward and backward, 882 us in
+// fp32 and 642 us in fp16 (20 and 27 TFLOP/s of what the recurrences need). As fp32 FMAs the same tiling took 1,205
 // and 1,176 us, held by shared memory's bandwidth.
 #include "launch.h"
 #include "linear_attn.cuh"

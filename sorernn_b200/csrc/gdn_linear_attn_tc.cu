@@ -9,7 +9,7 @@
 //   X <- a^nv X + U                  (fp32, in registers)
 // A, B and C are exact; the two-term splits of X, of W(P) and of the state's operand are good to 2^-17, so outputs are
 // within 2e-4 of RMS of their own rounding however slowly a head decays (X in one term left up to 0.018 of RMS more; its
-// second term costs the seventh product: a scan of the shape below 121 -> 141 us). A caller that gets the state itself
+// second term costs the seventh product, a scan of the shape below 121 -> 141 us). A caller that gets the state itself
 // (final state, gradient of the initial state) has its operand split in three (`precise`): fp32 accuracy. Two terms of a
 // 128 x 128 X do not fit beside the other tiles: its halves along DB, 32 KB of both terms, take turns in one place (the
 // staging tile in its stead, with outputs stored directly, made that 158 us).
@@ -23,15 +23,16 @@
 //   warps 12-15  the state: thread = a row of X^T, 128 fp32 registers (registers moved here with setmaxnreg)
 //   warps 16, 18, 19  issue the MMAs (P and Oa; U; Oi), each in uniform control flow with the issue predicated
 //   warp 17      issues the loads (single buffers; L2 prefetch two chunks ahead)
-// 8 x 4,096 tokens x 16 heads, DB = DC = 128: a scan takes 149 us, 4.7 us a chunk, 0.55 of a copy's rate over the four
-// tensors that it reads and writes; bound by the hand-overs between the roles and the products' shared-memory reads. The
-// fp32-accuracy kernel (gdn_linear_attn_fp32.cu) takes 903 us (64 features: 417 against 90; one chunk of 16 heads: 36
-// against 25 with the call), so bf16 runs here at every size that this one supports. The states-only form runs the split,
+// 8 x 4,096 tokens x 16 heads, DB = DC = 128: a scan takes 147 us, 4.6 us a chunk, 0.56 of a copy's rate over the four
+// tensors that it reads and writes; bound by the chain of hand-overs between the roles (tensor pipe 0.44 busy). The
+// fp32-accuracy kernel (gdn_linear_attn_fp32.cu) takes 903 us (64 features: 417 against 97; one chunk of 16 heads: 34
+// against 8), so bf16 runs here at every size that this one supports. The states-only form runs the split,
 // its product and the accumulator in two buffers each and loads B a whole chunk ahead: 2.1 us a chunk (159 us for the pieces
-// of 65,536 tokens x 16 heads with one buffer and half a chunk ahead, 118 so). What decided the layout with outputs,
+// of 65,536 tokens x 16 heads with one buffer and half a chunk ahead, 124 so). What decided the layout with outputs,
 // measured in the shape above (forward):
 //   * each role runs its code once a chunk, so the chunk loops have to fit the instruction cache together: 168 KB of
-//     unrolled code 12,800 cycles a chunk, 89 KB 6,900 (X in one term; X's terms written in two passes, 100 KB: 197 us);
+//     unrolled code 12,800 cycles a chunk, 89 KB 6,900 (X in one term; with two, a forward and backward took
+//     787 us with 100 KB, the terms written in two passes, and 670 with 90, the halves in turn);
 //   * an M = N = 128 product with both operands in shared memory takes nearly all of its read bandwidth (one every 65
 //     cycles): beside it a shared load of a warp's 512 bytes takes 60 cycles, a store 7, a global load 8. So the split
 //     reads B from global memory (L2) and the weights stay in registers.

@@ -2,8 +2,8 @@
 
 The arithmetic is fp32 with one rounding at the end: about eight operations of 2^-24 each on a value's path, the norm's sum
 included, on values of up to five RMS times weights of up to 1.8: 8 x 2^-24 x 9 = 4e-6 of RMS; 1e-5. Gradients subtract the
-mean of products of as many features again: 2e-5. What is left beyond half a unit in the last place of the type is measured, as
-in test_gpu_linear_attention_accuracy.py."""
+mean of products of as many features again: 2e-5. Measured is what is left beyond half a unit in the last place of the type,
+as in test_gpu_linear_attention_accuracy.py."""
 import pytest
 import torch
 
